@@ -447,8 +447,8 @@ typedef struct {
 
 /* Norm of every query and key head over head_dim, then the rotation of the pairs
  * (i, i + W/2) of each axis' W = head_dim / axes values by pos * base^(-2i/W) (axes 2, head
- * dim 64: m3s_vit_rope's layout).  Norm, angles (reduced in f64) and rotation in f32, one
- * rounding to dtype.  Rows of k_out / v_out outside [0, cache_rows) are dropped. */
+ * dim 64: m3s_vit_rope's layout).  Norm, angles (reduced in f64, of the f32 base; exact to f32
+ * for |pos| up to 2^38) and rotation in f32, one rounding to dtype.  Rows of k_out / v_out outside [0, cache_rows) are dropped. */
 int m3s_vit_qk_norm_rope(const m3s_qk_norm_rope_desc* desc, void* stream);
 
 typedef struct {

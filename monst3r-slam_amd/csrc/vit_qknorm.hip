@@ -18,7 +18,9 @@
 // wave: four that share a block's factors took 81 us.
 // Angles: revolutions in f64 (pos times the host's table of base^(-2i/W) / 2 pi), reduced to
 // [-1/2, 1/2] there and only then rounded to f32: an f32 angle of position 100,000 is off by
-// up to 2^-8 radians, this by 2^-24 of a half turn at any position below 2^40.
+// up to 2^-8 radians.  The table holds an f64 and what it leaves of the extended-precision value:
+// the f64 alone is off by 2^-24 of a half turn at positions of 2^30 and by 2^-15.5 at 2^40, the
+// pair by 2^-24 up to 2^38 and 2^-23.7 at 2^40 (base 100 to 500,000, against 113 bits).
 #include <math.h>
 #include "vit_common.h"
 
@@ -26,6 +28,7 @@ namespace {
 
 struct RevTable {
   double rev[64];   // revolutions per position step of pair i of an axis
+  float low[64];    // the value itself less rev
 };
 
 struct NormArgs {
@@ -132,7 +135,8 @@ __global__ __launch_bounds__(256, 3) void qk_norm_rope_kernel(NormArgs a, RevTab
     af[c] = g ? g[i & (D - 1)] : be ? 0.f : 1.f;
   }
   const int pa = lane % (D / 2) / half;
-  const double rev = rt.rev[lane % (D / 2) - pa * half];
+  const int pair = lane % (D / 2) - pa * half;
+  const double rev = rt.rev[pair], low = rt.low[pair];
   const uint32_t n = blockIdx.x * 4u + wave, n1 = min(n, a.tokens - 1);
   const int64_t b = n1 / (uint32_t)d.rows, s = n1 - (uint32_t)b * (uint32_t)d.rows;
   const int64_t p = d.pos[b * d.stride_pos + s * d.axes + pa];
@@ -143,8 +147,8 @@ __global__ __launch_bounds__(256, 3) void qk_norm_rope_kernel(NormArgs a, RevTab
 #pragma unroll
   for (int c = 0; c < AF; c++) (&affine[0][0][0])[c * 256 + tid] = af[c];
   if (lane < D / 2) {
-    double r = (double)p * rev;
-    r -= rint(r);
+    const double x = (double)p;
+    const double r = fma(x, low, fma(x, rev, -rint(x * rev)));
     float sn, c;
     sincospif((float)(2.0 * r), &sn, &c);
     tab[0][lane] = c;
@@ -200,7 +204,8 @@ extern "C" int m3s_vit_qk_norm_rope(const m3s_qk_norm_rope_desc* desc, void* str
   const int half = d.head_dim / d.axes / 2;
   const long double step = powl((long double)d.base, -1.0L / half);
   long double f = 1.0L / (2.0L * 3.14159265358979323846264338327950288L);
-  for (int i = 0; i < half; i++, f *= step) rt.rev[i] = (double)f;
+  for (int i = 0; i < half; i++, f *= step)
+    rt.rev[i] = (double)f, rt.low[i] = (float)(f - rt.rev[i]);
   hipStream_t s = m3s_stream(stream);
 #define M3S_NORM(T, D)                                                                     \
   hipLaunchKernelGGL((qk_norm_rope_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, a, rt)

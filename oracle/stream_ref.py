@@ -1,6 +1,7 @@
 """64-bit restatement of the streaming-layer operators (per-head norm + rotation, windowed
 attention over a cache, block-scaled e4m3), with the error that 32-bit sums and one rounding per
 result can make.  Plain torch on any device; the HIP kernels are tested against it."""
+import decimal
 import math
 
 import torch
@@ -15,8 +16,26 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def norm_rope(x, gamma, beta, pos, layer, eps, base):
-    """x [B, S, H, D], pos [B, S, axes] → (y f64, bound on the normed values per head f64)."""
+def angles(pos, half, base):
+    """pos base^(-i/half), whole turns taken off before the rounding to f64 (90 digits): f64
+    alone is off by position x 2^-53 radians.  pos [...] → f64 [..., half]."""
+    with decimal.localcontext() as c:
+        c.prec = 90
+        pi = decimal.Decimal("3.14159265358979323846264338327950288419716939937510"
+                             "58209749445923078164062862089986280348253421170680")
+        rev = [decimal.Decimal(base) ** (decimal.Decimal(-i) / half) / (2 * pi)
+               for i in range(half)]
+
+        def turn(p, r):
+            t = p * r
+            return float((t - t.to_integral_value()) * 2 * pi)
+        out = [[turn(int(p), r) for r in rev] for p in pos.reshape(-1).tolist()]
+    return torch.tensor(out, dtype=F64, device=pos.device).reshape(*pos.shape, half)
+
+
+def norm_rope(x, gamma, beta, pos, layer, eps, base, t=None):
+    """x [B, S, H, D], pos [B, S, axes] → (y f64, bound on the normed values per head f64).  t:
+    angles [B, S, axes, D / axes / 2] instead of f64's own (angles())."""
     x = x.to(F64)
     D, axes = x.shape[-1], pos.shape[-1]
     if layer:
@@ -27,8 +46,10 @@ def norm_rope(x, gamma, beta, pos, layer, eps, base):
     if beta is not None:
         y = y + beta.to(F64)
     half = D // axes // 2
-    inv = torch.tensor([base ** (-i / half) for i in range(half)], dtype=F64, device=x.device)
-    t = (pos.to(F64)[..., None] * inv)[:, :, None]           # [B, S, 1, axes, half]
+    if t is None:
+        inv = torch.tensor([base ** (-i / half) for i in range(half)], dtype=F64, device=x.device)
+        t = pos.to(F64)[..., None] * inv
+    t = t[:, :, None]                                        # [B, S, 1, axes, half]
     u, w = y.reshape(*y.shape[:-1], axes, 2, half).unbind(-2)
     out = torch.stack([u * t.cos() - w * t.sin(), w * t.cos() + u * t.sin()], -2)
     return out.flatten(-3), y.abs().amax(-1, keepdim=True).expand_as(y)

@@ -5,6 +5,7 @@ import math
 import os
 import shutil
 import subprocess
+from fractions import Fraction
 
 import pytest
 import torch
@@ -202,3 +203,19 @@ def test_descriptor_pack():
         big[[t for _, t in c._fields_].index(ctypes.c_int32)] = 1 << 31
         with pytest.raises(RuntimeError, match="out of range"):
             c.pack(*big)
+
+
+def test_angles():
+    """f64's own angles where f64 is exact enough, in [-pi, pi]; one that cancels to 6e-5 (710
+    is nearly 113 turns) keeps its digits."""
+    pos = torch.tensor([[0], [1], [-7], [3000], [1 << 20]])
+    t = R.angles(pos, 16, 100.0)
+    f = pos.double()[..., None] * torch.tensor([100.0 ** (-i / 16) for i in range(16)],
+                                               dtype=torch.float64)
+    # a product and a table entry rounded to 53 bits each, and the reduction's own
+    assert ((t.cos() - f.cos()).abs() <= 2.0 ** -51 * f.abs().clamp_min(1)).all()
+    assert ((t.sin() - f.sin()).abs() <= 2.0 ** -51 * f.abs().clamp_min(1)).all()
+    assert (t.abs() <= math.pi).all()
+    # math.sin(math.pi) is what math.pi lacks of pi
+    left = 710 - 226 * (Fraction(math.pi) + Fraction(math.sin(math.pi)))
+    assert abs(float(R.angles(torch.tensor([710]), 1, 1.0)) - float(left)) < 1e-18
