@@ -198,11 +198,12 @@ __device__ __forceinline__ void store_tile(const GArgs& a, const float* cs, int 
   const bool all = !a.vec;
   const int edge = all ? 0 : (a.N - n0) / 8 * 8;
   const int width = min(a.N - n0, COLS) - edge;
-  // with a.vec only the threads of the cut chunk are here: they walk its columns themselves
+  // with a.vec the threads of the cut chunk walk its columns themselves, and those whose chunks
+  // lie behind it have none (R may be C: an element is read and written by one thread)
   const int c1 = all ? tid % COLS : edge, r1 = all ? tid / COLS : r0;
   const int step = all ? NT / COLS : NT / TPR;
   const int last = all ? c1 + 1 : edge + width;
-  if (n0 + c1 >= a.N) return;
+  if (n0 + c1 >= a.N || (!all && c != edge)) return;
 #pragma unroll 1
   for (int cc = c1; cc < last; cc++) {
     const float bias = a.bias ? a.bias[n0 + cc] : 0.f;

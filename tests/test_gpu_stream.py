@@ -473,6 +473,26 @@ def test_gemm_block_residual_in_place_and_not_finite(ops, dev):
     _within(c[rows], ref[rows], tol[rows])
 
 
+@pytest.mark.parametrize("M,N,K", [(40, 60, 256), (300, 260, 272), (700, 1036, 640),
+                                   (700, 2100, 400), (1200, 2100, 144), (3300, 3100, 384)])
+def test_gemm_block_residual_in_place_at_a_cut_chunk(ops, dev, M, N, K):
+    """Columns that end inside a chunk of 8, rows aligned: R as C on every tile kernel, and 16-bit
+    rows of a padded C."""
+    rand = _gen(dev, N)
+    a, b = ((90 * rand(r, K)).clamp(-448, 448).to(torch.float8_e4m3fn) for r in (M, N))
+    G = -(-K // 128)
+    sa, sb = torch.exp(rand(G, M)) / 90, torch.exp(rand(-(-N // 128), G)) / (90 * K ** 0.5)
+    bias, c = rand(N), 3 * rand(M, N)
+    wide = torch.full((M, N + 4), 5.0, dtype=BF16, device=dev)
+    ops.gemm_block(a, sa, b, sb, wide[:, :N], bias=bias, R=c)
+    ref, tol = R.gemm_block(a, sa, b, sb, bias, False, c, BF16)
+    _within(wide[:, :N], ref, tol, "16-bit")
+    assert (wide[:, N:] == 5).all()
+    ref, tol = R.gemm_block(a, sa, b, sb, bias, False, c, F32)
+    ops.gemm_block(a, sa, b, sb, c, bias=bias, R=c)
+    _within(c, ref, tol, "in place")
+
+
 def test_gemm_block_deterministic(ops, dev):
     rand = _gen(dev, 33)
     M, N, K = 40, 512, 4096
