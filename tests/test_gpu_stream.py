@@ -454,6 +454,60 @@ def test_gemm_block_large_tiles(ops, dev, M, N, K):
     _gemm_case(ops, dev, M, N, K, F32, False, True, True)
 
 
+@pytest.mark.parametrize("K", [16, 128, 208, 256, 384, 512, 592, 640])
+def test_gemm_block_256_tiles(ops, dev, K):
+    """From 160 tiles of 256 x 256 on the two-group kernel takes over: one to five K-tiles, a cut
+    one, odd and even counts, cut rows and columns, aligned rows and others."""
+    _gemm_case(ops, dev, 3300, 3104, K, BF16, True, False, False, seed=K)
+    _gemm_case(ops, dev, 3300, 3101, K, F16, True, True, False, seed=K + 1)
+    _gemm_case(ops, dev, 3073, 3200, K, F32, False, False, True, seed=K + 2)
+
+
+@pytest.mark.parametrize("bias,gelu,res", [(True, True, True), (True, False, True),
+                                           (False, True, False), (False, False, False)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gemm_block_256_tiles_epilogues(ops, dev, bias, gelu, res, dtype):
+    """Every operand a view with strides of its own; then bias, residual and results that are not
+    16-B aligned."""
+    M, N, K = 2600, 4100, 272                            # 11 x 17 tiles
+    _gemm_case(ops, dev, M, N, K, dtype, bias, gelu, res, seed=1, pad=16)
+    rand = _gen(dev, 77)
+    a, b = ((90 * rand(r, K)).clamp(-448, 448).to(torch.float8_e4m3fn) for r in (M, N))
+    sa, sb = torch.rand(3, M + 7, device=dev)[:, 5:M + 5], torch.rand(33, 5, device=dev)[:, :3]
+    wide = torch.full((M, N + 5), 5.0, dtype=dtype, device=dev)
+    bi = rand(N + 3)[3:] if bias else None
+    R_ = rand(M, N + 1)[:, 1:] if res else None
+    ops.gemm_block(a, sa / 9e3, b, sb, wide[:, 3:N + 3], bias=bi, R=R_, gelu=gelu)
+    ref, tol = R.gemm_block(a, sa / 9e3, b, sb, bi, gelu, R_, dtype)
+    _within(wide[:, 3:N + 3], ref, tol)
+    assert (wide[:, :3] == 5).all() and (wide[:, N + 3:] == 5).all()
+
+
+@pytest.mark.parametrize("M,N", [(17, 40_961), (100, 41_000), (257, 20_500), (41_000, 40)])
+def test_gemm_block_256_tiles_one_band(ops, dev, M, N):
+    """Few rows of many columns, and the other way round: bands that are mostly padding."""
+    _gemm_case(ops, dev, M, N, 400, BF16, True, False, False, seed=M)
+    _gemm_case(ops, dev, M, N, 256, F32, False, False, True, seed=M)
+
+
+def test_gemm_block_256_tiles_not_finite(ops, dev):
+    """A NaN factor or operand reaches its own row or column only."""
+    rand = _gen(dev, 78)
+    M, N, K = 3300, 3100, 640
+    a, b = ((90 * rand(r, K)).clamp(-448, 448).to(torch.float8_e4m3fn) for r in (M, N))
+    sa, sb = torch.rand(5, M, device=dev), torch.rand(25, 5, device=dev)
+    ref, tol = R.gemm_block(a, sa, b, sb, None, False, None, F32)
+    sa[1, 300], sa[4, 3299], sb[3, 2] = math.nan, math.nan, math.nan
+    a.view(torch.uint8)[700, 639], b.view(torch.uint8)[3099, 0] = 0x7f, 0x7f
+    c = torch.empty(M, N, device=dev)
+    ops.gemm_block(a, sa, b, sb, c)
+    bad = torch.zeros(M, N, dtype=torch.bool, device=dev)
+    bad[[300, 700, 3299]] = True
+    bad[:, 384:512], bad[:, 3099] = True, True
+    assert torch.equal(torch.isnan(c), bad)
+    _within(torch.where(bad, 0, c), torch.where(bad, 0, ref), tol)
+
+
 def test_gemm_block_residual_in_place_and_not_finite(ops, dev):
     """R may be C; a NaN scale (a group that held an Inf) makes its row NaN and no other."""
     rand = _gen(dev, 31)
