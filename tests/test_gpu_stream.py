@@ -508,6 +508,23 @@ def test_gemm_block_256_tiles_not_finite(ops, dev):
     _within(torch.where(bad, 0, c), torch.where(bad, 0, ref), tol)
 
 
+@pytest.mark.parametrize("K", [272, 1024, 4096])
+@pytest.mark.parametrize("M,N", [(8, 4000), (100, 500), (700, 1000), (700, 2100), (1200, 2100),
+                                 (3300, 3100)])
+def test_gemm_block_f32_rms(ops, dev, M, N, K):
+    """f32 results on each kernel: no sum but the instruction's own is kept in few bits."""
+    rand = _gen(dev, M + K)
+    G = -(-K // 128)
+    a, b = ((90 * rand(r, K)).clamp(-448, 448).to(torch.float8_e4m3fn) for r in (M, N))
+    sa, sb = torch.exp(rand(G, M)) / 90, torch.exp(rand(-(-N // 128), G)) / (90 * K ** 0.5)
+    c = torch.empty(M, N, device=dev)
+    ops.gemm_block(a, sa, b, sb, c)
+    ref, _ = R.gemm_block(a, sa, b, sb, None, False, None, F32)
+    rms = float((c.double() - ref).square().mean().sqrt() / ref.square().mean().sqrt())
+    print(f"rms {rms:.3g}")
+    assert rms <= R.GEMM_BLOCK_RMS
+
+
 def test_gemm_block_residual_in_place_and_not_finite(ops, dev):
     """R may be C; a NaN scale (a group that held an Inf) makes its row NaN and no other."""
     rand = _gen(dev, 31)

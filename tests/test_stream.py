@@ -219,3 +219,27 @@ def test_angles():
     # math.sin(math.pi) is what math.pi lacks of pi
     left = 710 - 226 * (Fraction(math.pi) + Fraction(math.sin(math.pi)))
     assert abs(float(R.angles(torch.tensor([710]), 1, 1.0)) - float(left)) < 1e-18
+
+
+@pytest.mark.parametrize("K", [272, 1024, 4096])
+def test_gemm_block_rms_tells_short_sums(K):
+    """The bound on the product's rms error holds for the matrix instruction's cut octets and
+    fails for a sum over the groups that is rounded to 14 bits."""
+    g = torch.Generator().manual_seed(K)
+    M, N, G = 24, 48, -(-K // 128)
+    a, b = ((90 * torch.randn(r, K, generator=g)).clamp(-448, 448).to(torch.float8_e4m3fn)
+            for r in (M, N))
+    sa = torch.exp(torch.randn(G, M, generator=g)) / 90
+    sb = torch.exp(torch.randn(1, G, generator=g)) / (90 * K ** 0.5)
+    ref, tol = R.gemm_block(a, sa, b, sb, None, False, None, torch.float32)
+    a, b, sa, sb = a.double(), b.double(), sa.double(), sb.double()
+    cut, short = torch.zeros_like(ref), torch.zeros_like(ref)
+    for i in range(G):
+        k = slice(128 * i, 128 * i + 128)
+        f = sa[i][:, None] * sb[0, i]
+        cut += R.cut_octets(a[:, k], b[:, k]) * f
+        m, e = torch.frexp(short + a[:, k] @ b[:, k].t() * f)
+        short = torch.ldexp(torch.round(m * 2.0 ** 14) * 2.0 ** -14, e)
+    rms = lambda x: float(x.square().mean().sqrt() / ref.square().mean().sqrt())  # noqa: E731
+    assert ((cut - ref).abs() <= tol).all()
+    assert rms(cut - ref) < R.GEMM_BLOCK_RMS < rms(short - ref)
