@@ -243,3 +243,14 @@ def test_gemm_block_rms_tells_short_sums(K):
     rms = lambda x: float(x.square().mean().sqrt() / ref.square().mean().sqrt())  # noqa: E731
     assert ((cut - ref).abs() <= tol).all()
     assert rms(cut - ref) < R.GEMM_BLOCK_RMS < rms(short - ref)
+
+
+def test_ops_follow_the_current_device(monkeypatch):
+    """A device without an index is the one that is current at the call, not at the first one."""
+    from monst3r_slam_amd.model import Ops
+    ops = Ops(torch.device("cuda"))
+    x, q, s = torch.zeros(4, 128), torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 4)
+    for i in (0, 1):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: i)
+        with pytest.raises(RuntimeError, match=f"cuda:{i} "):
+            ops.quant_block(x, q, s)
