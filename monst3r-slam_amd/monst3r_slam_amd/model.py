@@ -255,7 +255,7 @@ class Ops:
             sb, sr, sh, sd = t.stride()
             if sd == 1 and (sh == d or h <= 1):
                 # a stride of a dimension of one row / batch is never used
-                return t.data_ptr(), sr if r > 1 else max(h * d, sr), sb if b > 1 else 0
+                return t.data_ptr(), sr if r > 1 else h * d, sb if b > 1 else 0
         self._refuse(idx, what, t, f"{name} must be {dtype} {list(shape)} [batch, rows, heads, "
                               "head_dim] with its heads side by side in a row")
 
@@ -277,7 +277,7 @@ class Ops:
             sr, sc = t.stride()
             if sc == 1 or c <= 1:
                 # a stride of a dimension of one row is never used
-                return t.data_ptr(), sr if r > 1 else max(c, sr)
+                return t.data_ptr(), sr if r > 1 else c
         self._refuse(idx, what, t, why)
 
     def qk_norm_rope(self, q, k, pos, q_out, k_out, *, gamma_q=None, beta_q=None, gamma_k=None,

@@ -339,6 +339,28 @@ def test_window_attn_strides(ops, dev):
     assert (wide[:, :, 0] == 3).all() and (wide[:, :, h + 1] == 3).all()
 
 
+def test_one_row_views(ops, dev):
+    """One token of each sequence out of rows whose length suits nothing: the row stride of a
+    single row is not used."""
+    rand = _gen(dev, 14)
+    B, h, D, L = 3, 2, 64, 40
+    W = h * D + 4                                          # 132 a row, 264 a sequence
+    view = lambda x: x.as_strided((B, 1, h, D), (2 * W, W, D, 1))  # noqa: E731
+    wide = rand(B, 2, h * D + 4).bfloat16()
+    q, out = view(wide), torch.full((B, 2, h * D + 4), 7.0, dtype=BF16, device=dev)
+    k, v = rand(B, L, h, D).bfloat16(), rand(B, L, h, D).bfloat16()
+    want, got = torch.empty(B, 1, h, D, dtype=BF16, device=dev), view(out)
+    ops.window_attn(q.contiguous(), k, v, want, 9, sinks=2)
+    ops.window_attn(q, k, v, got, 9, sinks=2)
+    assert torch.equal(got, want) and (out[:, 1] == 7).all() and (out[:, 0, h * D:] == 7).all()
+    pos = torch.arange(B, device=dev).reshape(B, 1, 1)
+    wk, want_k = torch.empty_like(want), torch.empty_like(want)
+    ops.qk_norm_rope(q.contiguous(), k[:, :1], pos, want, want_k)
+    ops.qk_norm_rope(q, k[:, :1], pos, got, wk)
+    assert torch.equal(got, want) and torch.equal(wk, want_k)
+    assert (out[:, 1] == 7).all() and (out[:, 0, h * D:] == 7).all()
+
+
 def test_window_attn_cache_past_32_bits(ops, dev):
     """A cache of more than 2^32 bytes: the newest keys lie behind the 32-bit offsets."""
     L, h, D = 2_200_000, 8, 128
