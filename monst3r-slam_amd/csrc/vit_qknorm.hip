@@ -22,6 +22,7 @@
 // the f64 alone is off by 2^-24 of a half turn at positions of 2^30 and by 2^-15.5 at 2^40, the
 // pair by 2^-24 up to 2^38 and 2^-23.7 at 2^40 (base 100 to 500,000, against 113 bits).
 #include <math.h>
+#include <type_traits>
 #include "vit_common.h"
 
 namespace {
@@ -85,24 +86,38 @@ __global__ __launch_bounds__(256, 3) void qk_norm_rope_kernel(NormArgs a, RevTab
       if (h0 + u * HP >= heads) break;
       const int hk = h0 + u * HP + grp - d.heads_q;
       float x[2][8];
+      // x, centred for a LayerNorm, times scale; its mean square
+      auto stats = [&](float scale) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[0][i] = (float)xu[u][i], x[1][i] = (float)xw[u][i];
-      if (d.layer) {
-        float m = 0.f;
+        for (int i = 0; i < 8; i++)
+          x[0][i] = (float)xu[u][i] * scale, x[1][i] = (float)xw[u][i] * scale;
+        if (d.layer) {
+          float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) m += x[0][i] + x[1][i];
+          for (int i = 0; i < 8; i++) m += x[0][i] + x[1][i];
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-        m *= 1.0f / D;
+          for (int o = LPH / 2; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
+          m *= 1.0f / D;
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[0][i] -= m, x[1][i] -= m;
+          for (int i = 0; i < 8; i++) x[0][i] -= m, x[1][i] -= m;
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += x[0][i] * x[0][i] + x[1][i] * x[1][i];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        return ss * (1.0f / D);
+      };
+      float var = stats(1.f) + d.eps;
+      if constexpr (std::is_same<T, bf16_t>::value) {
+        // bf16 has f32's exponents: a head whose squares leave f32 (or whose sum does) is scaled
+        const bool out = !(var >= 0x1p-96f && var <= 0x1p126f);
+        if (__builtin_amdgcn_ballot_w64(out)) {   // wave-uniform: the shuffles need every lane
+          const float scale = !out ? 1.f : var < 0x1p-96f ? 0x1p80f : 0x1p-80f;
+          var = stats(scale) + d.eps * scale * scale;
+        }
       }
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) ss += x[0][i] * x[0][i] + x[1][i] * x[1][i];
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-      const float r = 1.0f / sqrtf(ss * (1.0f / D) + d.eps);
+      const float r = 1.0f / sqrtf(var);
       const float(&af)[2][D] = affine[hk < 0 ? 0 : 1];
 #pragma unroll
       for (int p = 0; p < 2; p++)

@@ -88,6 +88,28 @@ def test_norm_rope_positions_up_to_2_40(ops, dev, D, axes, base):
         _within(got, ref, _norm_tol(ref, amp, F16))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("layer", [False, True])
+def test_norm_rope_every_magnitude(ops, dev, D, layer):
+    """bf16 heads whose squares or sums leave f32's range, up and down, beside ordinary ones."""
+    rand = _gen(dev, D + layer)
+    # one magnitude a token, most of them beside others in the wave's other heads
+    for eps, low in ((0.0, -125), (1e-5, -100)):
+        e = torch.arange(low, 126, device=dev)
+        x = rand(1, len(e), 6, D) + 0.5
+        x[:, :, 1::2] *= torch.exp2(e.float())[:, None, None]
+        x = x.bfloat16()
+        assert torch.isfinite(x).all()
+        pos = torch.randint(0, 500, (len(e), 1), device=dev)
+        q_out = torch.empty_like(x)
+        k_out = torch.empty_like(x[:, :, 1:2])
+        ops.qk_norm_rope(x, x[:, :, 1:2], pos, q_out, k_out, layer=layer, eps=eps, base=100.0)
+        ref, amp = R.norm_rope(x, None, None, pos[None], layer, eps, 100.0)
+        # the restatement's eps is the call's, rounded to f32: 2^-24 of it
+        _within(q_out, ref, _norm_tol(ref, amp, BF16))
+        assert torch.equal(k_out, q_out[:, :, 1:2])
+
+
 def test_norm_rope_in_place_and_zero_rows(ops, dev):
     rand = _gen(dev, 6)
     qk = rand(1, 33, 6, 128).bfloat16()
