@@ -419,7 +419,8 @@ int m3s_vit_attention(const void* d_q, int64_t ld_q, int64_t stride_q, const voi
 
 /* ---- Streaming transformer layers (ABI 0.6): per-head query / key norm with the rotation,
  * windowed attention over a key / value cache, block-scaled e4m3 products.  `dtype`,
- * `x_type` and `out_type` are M3S_BF16, M3S_F32 or M3S_F16; sizes of zero are no work. ---- */
+ * `x_type` and `out_type` are M3S_BF16, M3S_F32 or M3S_F16; a batch, rows, M or N of zero are no
+ * work, as is a quantiser's K of zero (a product needs K >= 16). ---- */
 enum { M3S_BF16 = 0, M3S_F32 = 1, M3S_F16 = 2 };
 
 typedef struct {
@@ -496,7 +497,8 @@ typedef struct {
   void* C; int64_t ldc;                    /* [M][ldc] of out_type                         */
   const float* bias;                       /* f32 [N], optional                            */
   const float* R; int64_t ldr;             /* f32 residual [M][ldr], optional; may be C    */
-  int32_t M, N, K;                         /* K % 16 == 0; A, B 16-B aligned, lda, ldb % 16 == 0 */
+  int32_t M, N, K;                         /* K % 16 == 0, K > 0 (else M3S_ERR_INVALID_ARG);
+                                              A, B 16-B aligned, lda, ldb % 16 == 0        */
   int32_t out_type, gelu;                  /* gelu: exact-erf GELU after the bias          */
 } m3s_gemm_block_desc;
 

@@ -254,3 +254,20 @@ def test_ops_follow_the_current_device(monkeypatch):
         monkeypatch.setattr(torch.cuda, "current_device", lambda: i)
         with pytest.raises(RuntimeError, match=f"cuda:{i} "):
             ops.quant_block(x, q, s)
+
+
+def test_zero_sizes():
+    """What the header calls no work is, and what it refuses is refused."""
+    from monst3r_slam_amd import _lib
+    lib = _lib.load()
+    for kw in (dict(batch=0), dict(rows=0), dict(heads_q=0, heads_kv=0)):
+        assert _norm(**kw) == 0, kw
+    for kw in (dict(batch=0), dict(rows=0)):
+        assert _attn(**kw) == 0, kw
+    for m, k in ((0, 256), (8, 0)):
+        assert lib.m3s_vit_quant_block(P, 0, 256, P, 256, P, 8, m, k, 0, None) == 0
+    base = dict(A=P, lda=256, scale_a=P, ld_sa=8, B=P, ldb=256, scale_b=P, ld_sb=2, C=P, ldc=100,
+                M=8, N=100, K=256)
+    for kw, want in ((dict(M=0), 0), (dict(N=0), 0), (dict(K=0), -1), (dict(K=0, M=0), -1)):
+        d = _lib.GemmBlockDesc(**{**base, **kw})
+        assert lib.m3s_vit_gemm_block(ctypes.byref(d), None) == want, kw
