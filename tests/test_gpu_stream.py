@@ -347,6 +347,25 @@ def test_window_attn_infinite_scores(ops, dev):
     assert (o[0, 0] == 0).all() and (o[0, 1] == 3).all()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,S,L,hq,hk", [(4, 1, 9000, 8, 2), (1, 40, 5000, 4, 2),
+                                         (1, 2100, 2300, 4, 4), (4, 700, 900, 16, 8)])
+def test_window_attn_repeats_exactly(ops, dev, D, B, S, L, hq, hk):
+    """The same call gives the same bits on every launch shape, split over the grid or not, with
+    other work on the card."""
+    rand = _gen(dev, S + D)
+    q, k, v = (rand(B, *n, D).bfloat16() for n in ((S, hq), (L, hk), (L, hk)))
+    outs = [torch.empty_like(q) for _ in range(6)]
+    side, x = torch.cuda.Stream(dev), rand(1024, 1024)
+    torch.cuda.synchronize(dev)
+    for o in outs:
+        with torch.cuda.stream(side):
+            _ = x @ x
+        ops.window_attn(q, k, v, o, 600, sinks=70)
+    torch.cuda.synchronize(dev)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 def test_window_attn_strides(ops, dev):
     """Views of a fused projection, transposed batch order, a cache with wider rows."""
     rand = _gen(dev, 11)
