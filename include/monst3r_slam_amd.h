@@ -456,7 +456,7 @@ typedef struct {
   const void* q; int64_t ld_q, stride_q;   /* [batch][rows] rows, head h at column h * head_dim */
   const void* k; int64_t ld_k, stride_k;   /* [batch][cache_rows]                          */
   const void* v; int64_t ld_v, stride_v;   /* 16-B aligned, ld and strides % 8 == 0 (o: 8-B, % 4) */
-  void* o; int64_t ld_o, stride_o;         /* [batch][rows]                                */
+  void* o; int64_t ld_o, stride_o;         /* [batch][rows]; may be q itself               */
   const int32_t* q_len;    /* [batch], clamped to [0, rows]; rows past it stay as they were
                               (NULL: rows)                                                 */
   const int32_t* kv_len;   /* [batch], clamped to [0, cache_rows] (NULL: cache_rows); the

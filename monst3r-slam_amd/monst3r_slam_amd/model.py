@@ -331,7 +331,8 @@ class Ops:
         [B, S, Hq, D], k, v [B, cache, Hkv, D] (Hkv divides Hq).  Query row i of batch b is
         token kv_len[b] - q_len[b] + i; it sees its own frame of `frame` tokens (frame 1: keys up
         to itself), the window - 1 frames before it (window 0: all) and the first `sinks` tokens.
-        Rows i >= q_len[b] of o are left alone; the cache behind kv_len[b] is not read.
+        Rows i >= q_len[b] of o are left alone; the cache behind kv_len[b] is not read.  o may be
+        q; otherwise it must not overlap the inputs.
         scale None: D ** -0.5."""
         what = "window_attn"
         idx = self._index()
@@ -361,7 +362,7 @@ class Ops:
     def quant_block(self, x, q, scale, pow2=False):
         """x [M, K] (bf16, f16 or f32) → q e4m3 [M, K] (float8_e4m3fn or uint8) and scale f32
         [ceil(K / 128), M]: one scale per row and 128 columns, amax / 448 or (pow2) the power of
-        two at or above it.  K % 16 == 0."""
+        two at or above it.  K % 16 == 0.  The three must not overlap."""
         what = "quant_block"
         idx = self._index()
         rows, shape = self._rows, x.shape
@@ -380,9 +381,10 @@ class Ops:
     def gemm_block(self, A, scale_a, B, scale_b, C, *, bias=None, R=None, gelu=False):
         """C [M, N] (bf16, f16 or f32) = (A scale_a) (B scale_b)ᵀ + bias, GELU, + R: A e4m3
         [M, K] with scale_a f32 [ceil(K / 128), M] (quant_block), B e4m3 [N, K] with scale_b f32
-        [ceil(N / 128), ceil(K / 128)] (quant_e4m3_block), K a multiple of 16 and not 0.  R f32 [M, N] may be C.  The e4m3
-        matrix instruction adds 8 neighbouring products to 13 binary places behind the largest,
-        all further sums are f32: f32 results are off by 1.5e-5 of their rms on random factors."""
+        [ceil(N / 128), ceil(K / 128)] (quant_e4m3_block), K a multiple of 16 and not 0.  R f32
+        [M, N] may be C; otherwise C must not overlap an operand.  The e4m3 matrix instruction
+        adds 8 neighbouring products to 13 binary places behind the largest, all further sums are
+        f32: f32 results are off by 1.5e-5 of their rms on random factors."""
         what = "gemm_block"
         idx = self._index()
         rows, sa, sb = self._rows, A.shape, B.shape

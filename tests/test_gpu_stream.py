@@ -349,6 +349,22 @@ def test_window_attn_infinite_scores(ops, dev):
 
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("B,S,L,hq,hk", [(4, 1, 9000, 8, 2), (1, 40, 5000, 4, 2),
+                                         (1, 2100, 2300, 4, 4), (4, 700, 900, 16, 8),
+                                         (2, 1001, 3, 12, 4)])
+def test_window_attn_in_place(ops, dev, D, B, S, L, hq, hk):
+    """o may be q itself: a block's rows are read before any of them is written, also where they
+    see nothing (1,001 queries over 3 keys) and where rows past a length stay queries."""
+    rand = _gen(dev, S + D)
+    q, k, v = (rand(B, *n, D).bfloat16() for n in ((S, hq), (L, hk), (L, hk)))
+    n = torch.tensor([S - S // 3 * (b % 2) for b in range(B)], device=dev, dtype=torch.int32)
+    want = q.clone()
+    ops.window_attn(q, k, v, want, 600, sinks=70, q_len=n)
+    ops.window_attn(q, k, v, q, 600, sinks=70, q_len=n)
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,S,L,hq,hk", [(4, 1, 9000, 8, 2), (1, 40, 5000, 4, 2),
                                          (1, 2100, 2300, 4, 4), (4, 700, 900, 16, 8)])
 def test_window_attn_repeats_exactly(ops, dev, D, B, S, L, hq, hk):
     """The same call gives the same bits on every launch shape, split over the grid or not, with
