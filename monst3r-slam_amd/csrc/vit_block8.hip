@@ -254,17 +254,18 @@ __device__ __forceinline__ void tile_of(const GArgs& a, int& tm, int& tn) {
 // scale group) filled by LDS-DMA; group g takes the K-tiles g, g + KS, ... and the groups' sums
 // join in LDS.  (A K-tile of one group is a chain of barrier, LDS reads, matrix instructions and
 // FMAs.  With one block a CU a second group fills it, and the next K-tile's LDS reads run beside
-// this one's matrix instructions: 768 x 1024 x 4096 12.1 -> 10.7 us; what is left is a CU's DMA
-// rate, 64 + 64 rows of K bytes at about 35 a cycle.  With KS = 1 three blocks a CU do it, and
-// the pipeline's registers would take one of them away: 2000 x 2048 x 2048 13.7 us, 15.9 with.)
+// this one's matrix instructions; what is left is a CU's DMA rate: 768 x 1024 x K takes 0.205 us
+// more for each K-tile of 64 + 64 rows, 80 B/ns or 35 a cycle.  With KS = 1 three blocks a CU do
+// it, and the pipeline's registers would take one of them away.)
 // The 16x16x128 matrix instruction takes a whole group: weights on the accumulator rows,
 // activations on the lanes, so an accumulator quad belongs to one activation row and its group's
 // factor sA sB is one value per lane and 16-row tile: acc += factor * partial, four FMAs beside
 // the 32 cycles of the next matrix instruction.
 // The instruction's own sums are f32 between groups of 8 products; the 8 are cut off 13 binary
-// places behind the largest one's exponent.  On random e4m3 that is 1.5e-5 of the result (rms;
-// 32-bit sums 1e-7), 1/2500 of what rounding random factors to e4m3 leaves in it (3.8e-2), and
-// 16-bit results hide it; products through bf16, which would avoid it, run at half the rate.
+// places behind the largest one's exponent.  On random e4m3 that is 1.5e-5 of the result
+// (rms; a 32-bit product 1.1e-6), 1/2500 of what rounding random factors to e4m3 leaves in it
+// (3.8e-2), and 16-bit results hide it; products through bf16, which would avoid it, run at half
+// the rate.
 template <int BM, int BN, int WM, int WN, int NST, int KS>
 __global__ __launch_bounds__(WM* WN* KS * 64, 2) void gemm_block_kernel(GArgs a) {
   constexpr int GT = WM * WN * 64, NT = GT * KS;
@@ -441,10 +442,12 @@ __global__ __launch_bounds__(WM* WN* KS * 64, 2) void gemm_block_kernel(GArgs a)
 //    or more after its last read Q: group 1's reads end before barrier 2Q + 2, which group 0
 //    passes before it issues phase Q + 2.  (A0, B0, scales: issued 2t, read 2t + 2, refilled
 //    2t + 4; A1: 2t + 1, 2t + 3, 2t + 5; B1: 2t + 1, 2t + 4, 2t + 7.)
-//  * DMA issue is what a phase has to share out: a wave's DMA instructions go out 120-160 cycles
-//    apart (4 waves 34 B a cycle, 8 waves 50 of a CU's 64).  Hence B1 a K-tile ahead: 5 and 4
-//    instructions a phase.  With 7 and 2 a K-tile took 3300 cycles, with four phases of one
-//    quadrant 3500; its matrix instructions are 2048 a SIMD.
+//  * DMA issue is what a phase has to share out: a wave waits for each of its DMA instructions to
+//    go out.  Hence B1 a K-tile ahead: 5 and 4 instructions a phase, not 7 and 2.
+// Measured (8192 x 8192 x K, bf16): a K-tile takes 1.70 us, 3,230 cycles at the 1.9 GHz that random
+// operands leave (zeros: 1.38 us, 3,040 at 2.2 GHz); its matrix instructions are 2,048 a SIMD.
+// Prologue and result writes are 10-14 us a tile.  K = 4096: 255 us, 2.15 PF/s; K = 8192: 475 us,
+// 2.31 PF/s.
 __global__ __launch_bounds__(512, 1) void gemm_block_pp_kernel(GArgs a) {
   constexpr int HT = 128 * 128, BUFB = 3 * HT, B1 = 2 * BUFB, SC = B1 + 3 * HT;
   // 2 buffers of scales: 256 activation rows (waves 0-3), 2 weight blocks (wave 4), zeros
@@ -631,7 +634,7 @@ __global__ __launch_bounds__(512, 1) void gemm_block_pp_kernel(GArgs a) {
 // Few rows (M <= 16): the weights are streamed once from memory to registers, one 16-column tile
 // a block, K-tiles dealt to the block's W waves; no LDS but for the join of the waves' sums.
 // HBM / latency bound: UN K-tiles of loads are in flight per wave before the first product
-// (5 x 7168 x 1792: 5.4 us, 2.4 TB/s; 16 x 8192 x 4096: 10.8 us, 3.1 TB/s).
+// (5 x 7168 x 1792: 5.9 us, 2.2 TB/s; 16 x 8192 x 4096: 11.1 us, 3.0 TB/s).
 template <int W>
 __global__ __launch_bounds__(W * 64) void gemm_block_rows_kernel(GArgs a) {
   constexpr int UN = 4;
@@ -779,17 +782,21 @@ extern "C" int m3s_vit_gemm_block(const m3s_gemm_block_desc* desc, void* stream)
   a.vec = (uintptr_t)d.C % 16 == 0 && d.ldc % (16 / size) == 0 && (uintptr_t)d.bias % 16 == 0 &&
           (!d.R || ((uintptr_t)d.R % 16 == 0 && d.ldr % 4 == 0));
   hipStream_t s = m3s_stream(stream);
-  // Measured (graph replays): M <= 16 5 x 7168 x 1792 5.4 us against 6.2 on 32-row tiles.  W waves
-  // share the K-tiles: 4 up to 16 of them (8: 6.3 us), 8 above (1 x 1024 x 4096 4.9, 4: 6.9 us)
+  // Measured (graph replays on rotating inputs): M <= 16 5 x 7168 x 1792 6.2 us against 6.6 on
+  // 32-row tiles, 1 x 1024 x 4096 5.6 against 8.8 (16 x 8192 x 4096 the other way: 11.1, 10.0).  W
+  // waves share the K-tiles: 4 up to 16 of them (8: 7.2 us), 8 above (1 x 1024 x 4096 5.6, 4: 7.9)
   if (d.M <= 16) return groups > 16 ? launch_rows<8>(a, s) : launch_rows<4>(a, s);
-  // 256^2 tiles once they fill most of the chip: 4096^3 66 us (64 x 128 tiles about 120); with
-  // 96 of them 3000 x 2000 x 2048 takes 33 us, 22 on 64 x 128
+  // 256^2 tiles once they fill most of the chip: 4096^3 66 us (64 x 128 tiles 100), 224 tiles of
+  // 3500 x 4096 x 2048 36 (46); with 96 of them 3000 x 2000 x 2048 takes 32 us, 21 on 64 x 128.
+  // The rule counts tiles, not what they hold: close to 160 (3300 x 3100 x 2048 52 us) and on 17 to
+  // 100 rows of many columns (32 x 65,536 x 4096 82 us) 64 x 128 tiles are ahead (45 and 71), on
+  // 192 rows they are not (102, 88)
   if ((int64_t)m3s_div_up(d.M, 256) * m3s_div_up(d.N, 256) >= 160) return launch_pp(a, s);
   // Few tiles leave a CU one block: two K groups in it, on the smallest tiles that one round of
-  // the CUs holds (768 x 1024 x 4096, 192 tiles of 64^2: 10.7 us; one group 14.2, three 10.8, four
-  // 11.7, 64 x 128 15.1; 196 x 768 x 4096 on 32-row tiles 8.6, 64^2 10.1; 1536 x 1024 x 4096, 192
-  // tiles of 64 x 128: 15.6, 64^2 19.6, one group 21.0).  Enough tiles: 64 x 128, one group
-  // (768 x 4096 x 1024 9.4 us, two groups 12.8)
+  // the CUs holds (768 x 1024 x 4096, 192 tiles of 64^2: 11.5 us; one group 14.3, 64 x 128 15.8;
+  // 196 x 768 x 4096 on 32-row tiles 9.5, 64^2 11.1; 1536 x 1024 x 4096, 192 tiles of 64 x 128:
+  // 16.8, 64^2 21.1, one group 21.8).  Enough tiles: 64 x 128, one group (768 x 4096 x 1024 9.9 us,
+  // two groups 13.6; 2000 x 2048 x 2048 15.1, 19.5)
   const int64_t m64 = m3s_div_up(d.M, 64);
   const int64_t b64 = m64 * m3s_div_up(d.N, 64), b128 = m64 * m3s_div_up(d.N, 128);
   if (b64 <= 96) return launch_tile<32, 64, 1, 4, 4, 2>(a, s);

@@ -21,9 +21,10 @@
 // not finite reaches only the rows that see its key (fix_values).
 //
 // Measured (MI355X, head dim 128 on 4 key heads / 64 on 16): one token of 4 sequences over
-// 65,536 keys 108 us, 4.97 TB/s of K and V (a large copy reaches 4.93); a 768-token frame over
-// 6,912 keys 46 us; 2 x 8,192 tokens, window 2,048: 268 us, 0.82 PF/s, where matrix pipe and
-// exponentials run at the clock that the card's power leaves.
+// 65,536 keys 106 us, 5.1 TB/s of K and V (a large copy reaches 4.93); a 768-token frame over
+// 6,912 keys 44 us, matrix pipe busy 28 % and vector issue 54 % of a busy CU's cycles; 2 x 8,192
+// tokens (ragged), window 2,048: 263 us, 0.84 PF/s, 50 % and 52 %, CUs busy 80 % of the time at
+// 1.9 GHz (zeros: 2.2 GHz, 212 us).
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -34,7 +35,6 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T>
 struct Mat;
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(AW* KS * 64, WPS) void wattn_kernel(WArgs a) {
   // their way from the start: what a short call waits for most): matrix and vector instructions
   // overlap across the waves of a SIMD (other blocks, at other places of their tiles).  Dealing
   // K Q^T of the next tile out between the exponentials of this one, or 64 rows a wave, changed
-  // nothing: on inputs that fill the matrix pipe the card's power is the bound (the same call on
-  // zeros takes 4/5 of the time).
+  // nothing (random inputs hold the clock at 1.9 GHz; the same call on zeros has 2.2 and takes 4/5
+  // of the time).
   const Range wfirst = visible(a, ql, kv, min(rw0, R - 1) / G);
   const Range wlast = visible(a, ql, kv, min(rw0 + 31, R - 1) / G);
   auto work = [&](int j, auto mask_tag) __attribute__((always_inline)) {
@@ -628,12 +628,12 @@ Plan plan_of(const m3s_window_attention_desc& d) {
   const bool d64 = d.head_dim == 64;
   Plan p;
   // Up to 256 tiles of 32 rows, or one a key head (single tokens): a block each, 4 key splits
-  // (16 sequences x 40 tokens over 4,000 keys, 8 heads of 128: 47 us, 4 x 2 waves 51; 512 tokens
-  // over 4,096 keys, 12 heads of 64 on 4: 20 us, 2 x 6 waves 24).  Up to 256 blocks of 128 rows:
-  // many waves on few rows, 2 x 6 for D = 64 (a 768-token frame over 6,912 keys of 16 heads 46 us;
-  // 1 x 4 62, 4 x 1 105, 4 x 2 78, 2 x 4 49, 2 x 8 46), 4 x 2 for D = 128 (12 heads 52 us; 1 x 4
-  // 90, 2 x 2 92).  Above, 4 row waves and several blocks a CU (8,192 tokens, 16 heads, window
-  // 2,048, D = 128: 266 us; 4 x 2 326; from 288 blocks on the two are within 5 %).
+  // (16 sequences x 40 tokens over 4,000 keys, 8 heads of 128: 60-67 us, 4 x 2 waves 67; 512
+  // tokens over 4,096 keys, 12 heads of 64 on 4: 21.5 us, 2 x 6 waves 24.3).  Up to 256 blocks of
+  // 128 rows: many waves on few rows, 2 x 6 for D = 64 (a 768-token frame over 6,912 keys of 16
+  // heads 43 us; 1 x 4 59, 4 x 1 94), 4 x 2 for D = 128 (12 heads 55 us; 1 x 4 92, 4 x 1 159).
+  // Above, 4 row waves and several blocks a CU (8,192 tokens, 16 heads, window 2,048, D = 128:
+  // 152 us, 4 x 2 167; D = 64: 91, 2 x 6 140; two such sequences of 128 267, 4 x 2 312).
   if ((R + 31) / 32 * hb <= 256 || R <= 32) p.aw = 1, p.ks = 4;
   else if (b4 <= 256) p.aw = d64 ? 2 : 4, p.ks = d64 ? 6 : 2;
   else p.aw = 4, p.ks = 1;
@@ -647,7 +647,9 @@ Plan plan_of(const m3s_window_attention_desc& d) {
                                        std::min<int64_t>(d.sinks, d.cache_rows));
   }
   // blocks with key splits fill a CU: grid splits up to one block a CU, of four tiles a wave at
-  // least (8 sequences x 1 token, window 4,096: 8 splits 16.5 us, 16 17.4, 32 23.4)
+  // least (8 sequences x 1 token, window 4,096: 8 splits 16.3 us, 4 18.7, 16 17.3, 32 22.6; one to
+  // two blocks a CU are not split: 40 sequences over 4,096 keys of 8 heads 156 us, with 2 splits
+  // 143, but 20 of them 68, with 2 splits 81)
   const int64_t tiles = (keys + kt - 1) / kt, blocks = p.nqt * hb;
   int64_t splits = 1;
   if (p.ks > 1 && blocks <= 128)
