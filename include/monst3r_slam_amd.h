@@ -476,7 +476,7 @@ typedef struct {
  * frame f = floor(p / frame), over the keys j < min(kv_len, (f + 1) frame) with
  * j >= (f - window + 1) frame or j < sinks; a row without keys is 0.  Statistics and sums in
  * f32, probabilities rounded to dtype.  Values that are not finite reach only rows that see
- * them.  Deterministic.  Each call in flight needs a workspace of its own. */
+ * them, as Inf or NaN.  Deterministic.  Each call in flight needs a workspace of its own. */
 size_t m3s_vit_window_attention_workspace_bytes(const m3s_window_attention_desc* desc);
 int m3s_vit_window_attention(const m3s_window_attention_desc* desc, void* stream);
 

@@ -334,6 +334,40 @@ def test_window_attn_without_workspace(ops, dev, S, D):
     _within(o, ref, tol)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,S,L,hq,hk", [(2, 3, 900, 8, 2), (4, 320, 500, 16, 8),
+                                         (4, 700, 900, 16, 8)])
+def test_window_attn_not_finite_queries(ops, dev, D, B, S, L, hq, hk):
+    """NaN and Inf in a query make its own row and head NaN and leave its neighbours, which share
+    its tiles, as they are."""
+    rand = _gen(dev, S + D)
+    q, k, v = (rand(B, *n, D).bfloat16() for n in ((S, hq), (L, hk), (L, hk)))
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    ops.window_attn(q, k, v, want, 600, sinks=70)
+    bad = torch.zeros(B, S, hq, dtype=torch.bool, device=dev)
+    for b, s, h, x in ((0, 0, 0, math.nan), (1, S - 1, hq - 1, math.inf), (1, S // 2, 3, math.nan)):
+        q[b, s, h, 5], bad[b, s, h] = x, True
+    ops.window_attn(q, k, v, got, 600, sinks=70)
+    assert torch.isnan(got[bad]).all()
+    assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_norm_rope_not_finite(ops, dev, D):
+    """NaN and Inf stay in their own head."""
+    rand = _gen(dev, D)
+    q, k = rand(2, 9, 5, D).bfloat16(), rand(2, 9, 20, D).bfloat16()
+    pos = torch.arange(9, device=dev)[:, None]
+    want, got = [[torch.empty_like(t) for t in (q, k)] for _ in range(2)]
+    ops.qk_norm_rope(q, k, pos, *want)
+    q[0, 3, 4, 7], q[1, 0, 0, D - 1], k[1, 8, 19, 0] = math.nan, math.inf, -math.inf
+    ops.qk_norm_rope(q, k, pos, *got)
+    for x, w, g in ((q, want[0], got[0]), (k, want[1], got[1])):
+        bad = ~torch.isfinite(x).all(-1)
+        assert bad.any() and (~torch.isfinite(g[bad])).any(-1).all()
+        assert torch.equal(g[~bad], w[~bad])
+
+
 def test_window_attn_infinite_scores(ops, dev):
     """Scores of -inf for every key a row sees: 0, as for a row that sees none; one finite key
     among them takes all the weight."""
