@@ -688,6 +688,60 @@ def test_gemm_block_deterministic(ops, dev):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+# ---- offsets past 32 bits: more than 2^32 bytes of inputs and results; the last rows are held
+# against the restatement of those rows alone ------------------------------------------------
+
+def test_quant_and_gemm_past_32_bits(ops, dev):
+    rand = _gen(dev, 61)
+    M, K, N, last = 600_000, 8192, 64, slice(599_900, 600_000)
+    x = torch.zeros(M, K, dtype=BF16, device=dev)
+    x[last] = rand(100, K).bfloat16()
+    q, s = torch.empty(M, K, dtype=torch.float8_e4m3fn, device=dev), torch.empty(64, M, device=dev)
+    ops.quant_block(x, q, s)
+    rq, rs = R.quant_block(x[last], False)
+    assert torch.equal(q[last].float().double(), rq) and torch.equal(s[:, last].double(), rs)
+    del x
+    b = (90 * rand(N, K)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    sb = torch.rand(1, 64, device=dev) / 90
+    c = torch.empty(M, N, device=dev)
+    ops.gemm_block(q, s, b, sb, c)
+    ref, tol = R.gemm_block(q[last], s[:, last], b, sb, None, False, None, F32)
+    _within(c[last], ref, tol)
+    assert (c[:599_900] == 0).all()
+
+
+@pytest.mark.parametrize("vec", [True, False])
+def test_gemm_block_results_past_32_bits(ops, dev, vec):
+    rand = _gen(dev, 62)
+    M, N, K, last = 70_000, 33_000 + (not vec), 128, slice(69_900, 70_000)
+    a, b = ((90 * rand(r, K)).clamp(-448, 448).to(torch.float8_e4m3fn) for r in (M, N))
+    sa, sb = torch.rand(1, M, device=dev) / 90, torch.rand(-(-N // 128), 1, device=dev) / 90
+    c = torch.zeros(M, N, device=dev)
+    c[last] = rand(100, N)
+    ref, tol = R.gemm_block(a[last], sa[:, last], b, sb, None, False, c[last], F32)
+    ops.gemm_block(a, sa, b, sb, c, R=c)
+    _within(c[last], ref, tol)
+
+
+def test_norm_and_attention_rows_past_32_bits(ops, dev):
+    rand = _gen(dev, 63)
+    S, h, D, L = 2_200_000, 8, 128, 300
+    q = torch.zeros(1, S, h, D, dtype=BF16, device=dev)
+    q[:, -L:] = rand(1, L, h, D).bfloat16()
+    k, v = rand(1, L, 2, D).bfloat16(), rand(1, L, 2, D).bfloat16()
+    o = torch.full_like(q, 3.0)
+    ops.window_attn(q, k, v, o, 64, sinks=2)              # query S - L + j stands at key j
+    ref, tol = R.window_attn(q[:, -L:], k, v, o[:, -L:], 64, 2, 1, None, None, D ** -0.5)
+    _within(o[:, -L:], ref, tol)
+    assert (o[:, :-L] == 0).all()
+    pos = torch.arange(S, device=dev)[:, None]
+    ko = torch.empty_like(q)
+    ops.qk_norm_rope(q, q, pos, o, ko, base=10000.0)
+    ref, amp = R.norm_rope(q[:, -L:], None, None, pos[None, -L:], False, 1e-6, 10000.0)
+    _within(o[:, -L:], ref, _norm_tol(ref, amp, BF16))
+    assert torch.equal(ko, o) and (o[:, :-L] == 0).all()
+
+
 # ---- together ------------------------------------------------------------------------------
 
 class _Layer:
